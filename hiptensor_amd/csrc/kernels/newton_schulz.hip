@@ -5,15 +5,19 @@
 // What is held in which type, and why.  The products run on v_mfma_f32_16x16x32_f16 (f16 operands, f32 sums; bf16 operands
 // would lose a factor of 8).  Two roundings would otherwise dominate the result:
 //   * X itself.  A rounding of X is noise in all directions, and the iteration amplifies what lies in directions of small
-//     singular values by up to a per step (485 over five steps).  X is therefore held as hi + lo, two f16 (22 bits): the
-//     products see hi, the term a X sees both.  The products' own neglect of lo is harmless: what it adds to a
-//     direction is in proportion to the singular value there.
+//     singular values by up to a per step (485 over five steps).  X is therefore held as hi + lo, two f16 (22 bits): A is of hi, and
+//     the term a X sees both.  So must B X, or none of it: in a direction of small singular value B is small as a whole, but its diagonal
+//     part is not.  Where all of B X is of hi, what is missing (B lo) lies in directions of large singular values only, where nothing
+//     amplifies it, and is four times the rounding of X there; where the diagonal's part sees lo and B' X does not, it is a third of that for
+//     matrices whose A is near the identity, and diag(e) lo, noise in all directions, for those of few directions (rank 1: 5e-2 off at
+//     2 x 2, 6e-3 at 64 x 64 after five steps).  A matrix of one workgroup multiplies lo too, which costs it little; on tiles, where lo in the product would
+//     be half of the update again, the diagonal's part sees lo in the last two steps, behind which no noise grows by more than a.
 //   * The diagonals of A and B.  Near the end A is close to the identity, and b A + c A A, a X + B X cancel to a
 //     fraction of their terms.  A = diag(d) + A', B = diag(e) + B' with d, e in f32 and only A', B' rounded to f16:
-//         A A = A' A' + (d_i + d_j) A'_ij + delta_ij d_i^2,      a X + B X = (a + e_i) X + B' X_hi,
+//         A A = A' A' + (d_i + d_j) A'_ij + delta_ij d_i^2,      a X + B X = a X + e_i X + B' X,
 //     elementwise terms that the epilogues of the products add in f32.
-// On gaussian matrices the result is 5e-4 .. 1e-3 off (2-norm; 1e-3 .. 2e-3 with plain f16, 1e-2 with bf16), on low rank plus
-// 1 % noise 8e-4 (4e-2 with plain f16, 0.3 with bf16): below the rounding of a bf16 result, 1.7e-3.
+// On gaussian matrices the result is 5e-4 .. 1.1e-3 off (2-norm, five steps; 1e-3 .. 2e-3 with plain f16, 1e-2 with bf16), on low rank plus
+// 1 % noise 3e-4 .. 1e-3 (4e-2 with plain f16, 0.3 with bf16): below the rounding of a bf16 result, 1.7e-3.
 // All f16 matrices hold their values times 2^10: entries of X, A and B stay below 64 and keep full precision down to 2^-24.
 //
 // A' and B' are symmetric: tiles above the diagonal are mirrored, not multiplied.  B' X contracts the rows of
@@ -57,6 +61,7 @@ namespace
         int32_t     parts, lanes_log; // of the norm
         int32_t     type_x, type_o;
         float       a, b, c, epsilon;
+        float       e_lo; // how much of X_lo the diagonal of B multiplies: 1 in the last two steps, 0 before
     };
 
     template <typename T>
@@ -633,10 +638,10 @@ namespace
                     }
                     else
                     {
-                        const float f = a.a + of_q[s][it];
+                        const float f = a.a + of_q[s][it], g = a.a + a.e_lo * of_q[s][it];
 #pragma unroll
                         for(int h = 0; h < 8; h++)
-                            v[h] = f * ((float)one[s][it][h] + (float)two[s][it][h]) + v[h] * DOWN;
+                            v[h] = f * (float)one[s][it][h] + (g * (float)two[s][it][h] + v[h] * DOWN);
                         if constexpr(MODE == NS_UPDATE)
                         {
                             h8 low;
@@ -716,9 +721,10 @@ namespace
 
     // ---- matrices that one compute unit holds --------------------------------------------------------------------------
 
-    // The whole iteration of one matrix (padded to MP x NP) in one workgroup of eight wavefronts: X_hi and A' (then B') in LDS, X in f32 in the registers
+    // The whole iteration of one matrix (padded to MP x NP) in one workgroup of eight wavefronts: X_hi, X_lo and A' (then B') in LDS, X in f32 in the registers
     // of the lanes that update it, so that there is one launch instead of three a step (64 x 256: 65 us in 17 launches,
-    // 24 us so, 300 of them 37 us; most of it is the latency of LDS and barriers).  X_hi is read along n for X X^T and, by transposing reads, along m for B X.
+    // 24.5 us so, 300 of them 41 us; most of it is the latency of LDS and barriers).  X_hi is read along n for X X^T and, by transposing reads, along m for
+    // B X, as X_lo is (B X of X_hi alone: 22 and 36 us; of X_lo put in X_hi's place, as 128 x 256 has it, 26 and 43).
     struct Coefficients
     {
         static constexpr int MOST = 16; // steps
@@ -734,7 +740,9 @@ namespace
         static constexpr int SJ = SQ < 4 ? SQ : 4, SI = SQ / SJ; // (MB 4: 1 x 2; MB 8: 2 x 4)
         static constexpr int XB = MB * NBL / WAVES;             // blocks of X a wavefront: UI along n by UJ along m
         static constexpr int UJ = XB < MB ? XB : MB, UI = XB / UJ;
-        static constexpr int LDS = 2 * (MP * PX + MP * PA) + 4 * 2 * MP + 64;
+        static constexpr int  LEAST  = 2 * (MP * PX + MP * PA) + 4 * 2 * MP + 64;
+        static constexpr bool BESIDE = LEAST + 2 * MP * PX <= 160 * 1024; // X_lo has a place of its own (else X_hi's, when that has been read)
+        static constexpr int  LDS    = LEAST + (BESIDE ? 2 * MP * PX : 0);
         static_assert(MB * MB % WAVES == 0 && UI * UJ * WAVES == MB * NBL && MB % UJ == 0 && LDS <= 160 * 1024, "");
     };
 
@@ -744,7 +752,7 @@ namespace
         typedef Small<MP, NP> T;
         constexpr int PX = T::PX, PA = T::PA, SI = T::SI, SJ = T::SJ, UI = T::UI, UJ = T::UJ;
         extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-        _Float16 *      X = (_Float16*)lds, *A = X + MP * PX;
+        _Float16 *      X = (_Float16*)lds, *lower = T::BESIDE ? X + MP * PX : X, *A = lower + MP * PX;
         float *         d = (float*)(A + MP * PA), *e = d + MP;
         double*         part = (double*)(e + MP);
         const int       tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, fr = lane & 15, g = lane >> 4;
@@ -799,17 +807,27 @@ namespace
         for(int w = 0; w < T::WAVES; w++)
             s += part[w];
         const double factor = (double)UP / (sqrt(s) + (double)a.epsilon);
-        auto         put = [&]() __attribute__((always_inline)) {
+        auto low_of = [&](const f4& v) __attribute__((always_inline)) {
+            h4 h;
+#pragma unroll
+            for(int r = 0; r < 4; r++)
+                h[r] = (_Float16)(v[r] - (float)(_Float16)v[r]);
+            return h;
+        };
+        auto put = [&]() __attribute__((always_inline)) {
 #pragma unroll
             for(int i = 0; i < UI; i++)
 #pragma unroll
                 for(int j = 0; j < UJ; j++)
                 {
-                    h4 h;
+                    const int at = (16 * (uj + j) + fr) * PX + 16 * (ui + i) + 4 * g;
+                    h4        h;
 #pragma unroll
                     for(int r = 0; r < 4; r++)
                         h[r] = (_Float16)x[i][j][r];
-                    *(h4*)&X[(16 * (uj + j) + fr) * PX + 16 * (ui + i) + 4 * g] = h;
+                    *(h4*)&X[at] = h;
+                    if constexpr(T::BESIDE)
+                        *(h4*)&lower[at] = low_of(x[i][j]);
                 }
         };
 #pragma unroll
@@ -918,56 +936,99 @@ namespace
             __syncthreads();
             // X <- a X + B X
             // (in place: (a + e) X scaled as the products are, and back)
+            h4 low[T::BESIDE ? 1 : UI][T::BESIDE ? 1 : UJ];
 #pragma unroll
             for(int j = 0; j < UJ; j++)
             {
                 const float f = (ca + e[16 * (uj + j) + fr]) * UP;
 #pragma unroll
                 for(int i = 0; i < UI; i++)
+                {
+                    if constexpr(!T::BESIDE)
+                        low[i][j] = low_of(x[i][j]);
                     x[i][j] *= f;
+                }
             }
             typedef short s4 __attribute__((ext_vector_type(4)));
             typedef s4 __attribute__((address_space(3))) * s4_ptr;
             typedef _Float16 __attribute__((address_space(3))) * h_ptr;
-#pragma unroll
-            for(int k = 0; k < MP; k += 32)
-            {
-                h8 fp[UI], fq[UJ];
-#pragma unroll
-                for(int i = 0; i < UI; i++)
+            auto turned = [&](const _Float16* from, int k, int i) __attribute__((always_inline)) {
+                const h_ptr at = (h_ptr)from + (k + 8 * g + (fr >> 2)) * PX + 16 * (ui + i) + 4 * (fr & 3);
+                const uint2 u = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_ptr)at));
+                const uint2 v = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_ptr)(at + 4 * PX)));
+                return __builtin_bit_cast(h8, uint4{u.x, u.y, v.x, v.y});
+            };
+            auto product = [&](auto both_c) __attribute__((always_inline)) { // B' X_hi, or B' (X_hi + X_lo)
+                constexpr bool BOTH = decltype(both_c)::value;
+#pragma unroll 2
+                for(int k = 0; k < MP; k += 32)
                 {
-                    const h_ptr at = (h_ptr)X + (k + 8 * g + (fr >> 2)) * PX + 16 * (ui + i) + 4 * (fr & 3);
-                    const uint2 lo = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_ptr)at));
-                    const uint2 hi = __builtin_bit_cast(uint2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4_ptr)(at + 4 * PX)));
-                    fp[i]          = __builtin_bit_cast(h8, uint4{lo.x, lo.y, hi.x, hi.y});
-                }
+                    h8 fp[UI], fl[UI], fq[UJ];
 #pragma unroll
-                for(int j = 0; j < UJ; j++)
-                    fq[j] = *(const h8*)&A[(16 * (uj + j) + fr) * PA + k + 8 * g];
+                    for(int i = 0; i < UI; i++)
+                    {
+                        fp[i] = turned(X, k, i);
+                        if constexpr(BOTH)
+                            fl[i] = turned(lower, k, i);
+                    }
+#pragma unroll
+                    for(int j = 0; j < UJ; j++)
+                        fq[j] = *(const h8*)&A[(16 * (uj + j) + fr) * PA + k + 8 * g];
+#pragma unroll
+                    for(int i = 0; i < UI; i++)
+#pragma unroll
+                        for(int j = 0; j < UJ; j++)
+                            x[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[i], fq[j], x[i][j], 0, 0, 0);
+                    if constexpr(BOTH)
+                    {
+#pragma unroll
+                        for(int i = 0; i < UI; i++)
+#pragma unroll
+                            for(int j = 0; j < UJ; j++)
+                                x[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fl[i], fq[j], x[i][j], 0, 0, 0);
+                    }
+                }
+            };
+            if constexpr(T::BESIDE)
+                product(std::true_type{});
+            else
+            {
+                // (a wavefront holds all of m here: the columns of X_hi that it reads are its own, and LDS serves a wavefront in order)
+                static_assert(UJ == T::MB, "");
+                auto in_order = [&]() __attribute__((always_inline)) {
+                    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+                    __builtin_amdgcn_wave_barrier();
+                };
+                product(std::false_type{});
+                in_order();
 #pragma unroll
                 for(int i = 0; i < UI; i++)
 #pragma unroll
                     for(int j = 0; j < UJ; j++)
-                        x[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fp[i], fq[j], x[i][j], 0, 0, 0);
+                        *(h4*)&X[(16 * (uj + j) + fr) * PX + 16 * (ui + i) + 4 * g] = low[i][j];
+                in_order();
+                product(std::false_type{});
             }
 #pragma unroll
             for(int i = 0; i < UI; i++)
 #pragma unroll
                 for(int j = 0; j < UJ; j++)
                     x[i][j] *= DOWN;
-            __syncthreads(); // (X_hi, B' and e have been read)
+            __syncthreads(); // (X_hi, X_lo, B' and e have been read)
             if(step + 1 < steps)
             {
                 put();
                 __syncthreads();
             }
         }
+        int last_fr = fr, last_g = g;
+        asm volatile("" : "+v"(last_fr), "+v"(last_g)); // (what O's addresses share with X's is not kept in registers through the steps)
 #pragma unroll
         for(int i = 0; i < UI; i++)
 #pragma unroll
             for(int j = 0; j < UJ; j++)
             {
-                const int     m = 16 * (uj + j) + fr, n = 16 * (ui + i) + 4 * g;
+                const int     m = 16 * (uj + j) + last_fr, n = 16 * (ui + i) + 4 * last_g;
                 const int64_t at = (int64_t)z * a.stride_o + (a.tall ? (int64_t)n * a.ldo + m : (int64_t)m * a.ldo + n);
                 any_h4        h;
 #pragma unroll
@@ -1244,6 +1305,7 @@ extern "C" int hiptk_orthogonalize(const hiptk_orthogonalize_t* p, void* workspa
         a.a              = abc[0];
         a.b              = abc[1];
         a.c              = abc[2];
+        a.e_lo           = s + 2 >= p->steps ? 1.f : 0.f;
         a.hi             = (_Float16*)(ws + (s & 1 ? l.next : l.hi));
         a.hi_out         = (_Float16*)(ws + (s & 1 ? l.hi : l.next));
         if(l.slices > 1)

@@ -1,0 +1,49 @@
+"""Orthogonalisation where roundings have most to say: matrices of few directions, which the iteration amplifies what it leaves
+in the others of, and equal rows or entries, whose roundings do not average out.  Results in f16, which hide least."""
+import pytest
+import torch
+
+import layer_ops as L
+
+pytestmark = pytest.mark.gpu
+
+
+def bound(rows, cols, steps, repeats, out):
+    """The error that the header allows, and one rounding to the result's type."""
+    base = 3e-3 if steps <= 6 else 6e-3
+    few = 4 if repeats or min(rows, cols) < 16 else 1
+    return base * few + 2.0**-23 * L.COEFFICIENTS[0]**steps + L.ROUND[out][0]
+
+
+def matrix(kind, rows, cols, seed):
+    g = torch.Generator().manual_seed(1000 * rows + cols + seed)
+    new = lambda *s: torch.randn(*s, generator=g)  # noqa: E731
+    if kind.startswith("rank"):
+        r = min(int(kind.split()[1]), rows, cols)
+        return new(rows, r) @ new(r, cols)
+    if kind == "low rank and noise":
+        return new(rows, 8) @ new(8, cols) + 1e-3 * new(rows, cols)
+    if kind == "one direction above noise":
+        return new(rows, cols) + 30 * new(rows, 1) @ new(1, cols)
+    if kind == "two equal rows":
+        x = torch.zeros(rows, cols)
+        x[0] = x[-1] = new(cols)
+        return x
+    if kind == "equal entries":
+        return torch.full((rows, cols), 0.37)
+    return new(rows, cols)
+
+
+# one workgroup a matrix; products on tiles
+SHAPES = [(2, 2), (2, 4), (8, 64), (64, 8), (64, 64), (30, 500), (100, 128), (128, 256), (250, 100),
+          (2, 600), (33, 600), (600, 33), (64, 520), (130, 520), (300, 700), (700, 300)]
+
+
+@pytest.mark.parametrize("rows,cols", SHAPES)
+@pytest.mark.parametrize("kind", ["rank 1", "rank 2", "rank 4", "low rank and noise", "one direction above noise", "two equal rows", "equal entries"])
+def test_few_directions(gpu_handle, rows, cols, kind):
+    x = torch.stack([matrix(kind, rows, cols, seed) for seed in range(4)])
+    got, want = L.gpu_orthogonalize(gpu_handle, x, "f32", "f16"), L.orthogonalize_plain(x, 5)
+    for i in range(4):
+        off = L.relative(got[i], want[i])
+        assert off <= bound(rows, cols, 5, "equal" in kind, "f16"), (i, off)
