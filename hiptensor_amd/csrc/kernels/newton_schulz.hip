@@ -723,8 +723,8 @@ namespace
 
     // The whole iteration of one matrix (padded to MP x NP) in one workgroup of eight wavefronts: X_hi, X_lo and A' (then B') in LDS, X in f32 in the registers
     // of the lanes that update it, so that there is one launch instead of three a step (64 x 256: 65 us in 17 launches,
-    // 24.5 us so, 300 of them 41 us; most of it is the latency of LDS and barriers).  X_hi is read along n for X X^T and, by transposing reads, along m for
-    // B X, as X_lo is (B X of X_hi alone: 22 and 36 us; of X_lo put in X_hi's place, as 128 x 256 has it, 26 and 43).
+    // 21 us so, 300 of them 36 us; most of it is the latency of LDS and barriers).  X_hi is read along n for X X^T and, by transposing reads, along m for
+    // B X, as X_lo is.
     struct Coefficients
     {
         static constexpr int MOST = 16; // steps
@@ -834,9 +834,14 @@ namespace
         for(int i = 0; i < UI; i++)
 #pragma unroll
             for(int j = 0; j < UJ; j++)
+            {
 #pragma unroll
                 for(int r = 0; r < 4; r++)
                     x[i][j][r] = (float)((double)x[i][j][r] * factor); // (the padding's zeros too: a factor that is not finite makes the matrix NaN as it is)
+                // (X_hi is of this f32, as X_lo is: left to itself the compiler rounds the f64 product to X_hi in one step, which is
+                // another f16 where the f32 lies halfway between two, and X_hi + X_lo would not be X there)
+                asm volatile("" : "+v"(x[i][j]));
+            }
         put();
         __syncthreads();
 

@@ -47,3 +47,25 @@ def test_few_directions(gpu_handle, rows, cols, kind):
     for i in range(4):
         off = L.relative(got[i], want[i])
         assert off <= bound(rows, cols, 5, "equal" in kind, "f16"), (i, off)
+
+
+@pytest.mark.parametrize("rows,cols", [(2, 4), (8, 64), (64, 64), (128, 256), (100, 50), (33, 600), (300, 200), (512, 512)])
+@pytest.mark.parametrize("kind", ["gaussian", "rank 1", "low rank and noise", "two equal rows"])
+@pytest.mark.parametrize("steps", [1, 2, 3, 6, 8, 10, 12])
+def test_steps(gpu_handle, rows, cols, kind, steps):
+    """Results of odd and even numbers of steps, and of more than the usual five or six."""
+    x = torch.stack([matrix(kind, rows, cols, 10 + seed) for seed in range(2)])
+    got, want = L.gpu_orthogonalize(gpu_handle, x, "f32", "f16", steps), L.orthogonalize_plain(x, steps)
+    for i in range(2):
+        off = L.relative(got[i], want[i])
+        assert off <= bound(rows, cols, steps, "equal" in kind, "f16"), (i, off)
+
+
+@pytest.mark.parametrize("rows,cols", [(60, 100), (100, 60), (40, 700)])
+def test_steps_that_converge(gpu_handle, rows, cols):
+    """Coefficients whose error does not grow, and more steps than one launch of a small matrix holds."""
+    coefficients = [1.875, -1.25, 0.375]
+    x = torch.stack([matrix("gaussian", rows, cols, 20 + seed) for seed in range(2)])
+    for steps in (16, 17, 30):
+        got, want = L.gpu_orthogonalize(gpu_handle, x, "f32", "f16", steps, coefficients * steps), L.orthogonalize_plain(x, steps, coefficients * steps)
+        assert L.relative(got, want) <= 3e-3 + L.ROUND["f16"][0], steps
