@@ -18,7 +18,8 @@
 //     elementwise terms that the epilogues of the products add in f32.
 // On gaussian matrices the result is 5e-4 .. 1.1e-3 off (2-norm, five steps; 1e-3 .. 2e-3 with plain f16, 1e-2 with bf16), on low rank plus
 // 1 % noise 3e-4 .. 1e-3 (4e-2 with plain f16, 0.3 with bf16): below the rounding of a bf16 result, 1.7e-3.
-// All f16 matrices hold their values times 2^10: entries of X, A and B stay below 64 and keep full precision down to 2^-24.
+// X is held times 2^10, A' and B' times the power of two up to 2^10 that what a call's coefficients can make of them leaves (Scales): the default ones leave
+// 2^10, entries stay below 64 and keep full precision down to 2^-24.
 //
 // A' and B' are symmetric: tiles above the diagonal are mirrored, not multiplied.  B' X contracts the rows of
 // X_hi: its tiles go into LDS as they lie, row by row, and the reads from there transpose.  All dimensions are padded to multiples of 64 with zeros,
@@ -42,6 +43,52 @@ namespace
     constexpr float DEFAULT_COEFFICIENTS[3] = {3.4445f, -4.7750f, 2.0315f};
     constexpr float UP = 1024.f, DOWN = 1.f / 1024.f;
 
+    // What the f16 A' and B' of all steps are held times.  No entry of a matrix is larger than its largest singular value: with those of X up to `most`
+    // (1 at first: X / |X|_F), A's are t = s^2 up to most^2, B's |b t + c t^2|, and those of the next X s |a + b t + c t^2|, largest at the end of
+    // the range or where the derivative is zero.  (The iterates of a call's coefficients stay below MOST_X by the interface, which X's own scale needs,
+    // whatever this bound for any matrix says.  One pair for all steps: read anew in each, it cost a 64 x 64 matrix 0.8 of 10.8 us.)
+    struct Scales
+    {
+        float up_a, down_a, up_b, down_b;
+    };
+    constexpr double MOST_X = 16.0;
+    Scales           scales_of(const float* coefficients, int steps)
+    {
+        if(!coefficients)
+            return Scales{UP, DOWN, UP, DOWN}; // (from [0, 1.21] back into it, B up to 2.81)
+        double most = 1.0, most_a = 0.0, most_b = 0.0;
+        for(int s = 0; s < steps; s++)
+        {
+            const double a = coefficients[3 * s], b = coefficients[3 * s + 1], c = coefficients[3 * s + 2], end = most * most;
+            double       peak_b = 0.0, peak_x = 0.0;
+            auto         at     = [&](double t) { // (a t that is not a number is not in the range)
+                if(t > 0.0 && t <= end)
+                {
+                    const double v = t * (b + c * t);
+                    peak_b         = __builtin_fmax(peak_b, __builtin_fabs(v));
+                    peak_x         = __builtin_fmax(peak_x, __builtin_sqrt(t) * __builtin_fabs(a + v));
+                }
+            };
+            const double root = __builtin_sqrt(9.0 * b * b - 20.0 * a * c); // of a + 3 b t + 5 c t^2
+            at(end);
+            at(-b / (2.0 * c));
+            at((-3.0 * b - root) / (10.0 * c));
+            at((-3.0 * b + root) / (10.0 * c));
+            at(-a / (3.0 * b)); // (c = 0)
+            most_a = __builtin_fmax(most_a, end);
+            most_b = __builtin_fmax(most_b, peak_b);
+            most   = peak_x < MOST_X ? peak_x : MOST_X;
+        }
+        auto up = [](double peak) { // the largest power of two that keeps peak, and its roundings, within f16 (of a peak that is not finite the smallest)
+            double u = UP;
+            while(!(peak * u <= 60000.0) && u > 0x1p-100)
+                u *= 0.5;
+            return (float)u;
+        };
+        const float ua = up(most_a), ub = up(most_b);
+        return Scales{ua, 1.f / ua, ub, 1.f / ub};
+    }
+
     struct NsArgs
     {
         _Float16 *hi, *lo;     // X, [m][n]
@@ -61,6 +108,7 @@ namespace
         int32_t     parts, lanes_log; // of the norm
         int32_t     type_x, type_o;
         float       a, b, c, epsilon;
+        Scales      scales;
         float       e_lo; // how much of X_lo the diagonal of B multiplies: 1 in the last two steps, 0 before
     };
 
@@ -607,16 +655,17 @@ namespace
                     uint16_t bits[8];
                     if constexpr(!UPDATE)
                     {
+                        const float    down_a = a.scales.down_a, up = SQUARE ? a.scales.up_a : a.scales.up_b;
                         const float    dq   = MODE == NS_MIX ? of_q[s][it] : 0.f;
                         const uint32_t diag = (uint32_t)(q - pc); // the chunk's element on the diagonal, if less than 8
 #pragma unroll
                         for(int h = 0; h < 8; h++)
                         {
-                            v[h] *= DOWN * DOWN;
+                            v[h] *= SQUARE ? DOWN * DOWN : down_a * down_a;
                             if constexpr(MODE == NS_MIX)
                             {
                                 // (on the diagonal A' is zero, and d_i^2 is added to A A, d_i to A below)
-                                const float off = (float)one[s][it][h] * DOWN;
+                                const float off = (float)one[s][it][h] * down_a;
                                 v[h]            = a.b * off + a.c * (v[h] + (dp[it][h / 4][h % 4] + dq) * off);
                             }
                         }
@@ -634,14 +683,14 @@ namespace
                         }
 #pragma unroll
                         for(int h = 0; h < 8; h++)
-                            bits[h] = __builtin_bit_cast(uint16_t, (_Float16)(v[h] * UP));
+                            bits[h] = __builtin_bit_cast(uint16_t, (_Float16)(v[h] * up));
                     }
                     else
                     {
                         const float f = a.a + of_q[s][it], g = a.a + a.e_lo * of_q[s][it];
 #pragma unroll
                         for(int h = 0; h < 8; h++)
-                            v[h] = f * (float)one[s][it][h] + (g * (float)two[s][it][h] + v[h] * DOWN);
+                            v[h] = f * (float)one[s][it][h] + (g * (float)two[s][it][h] + v[h] * a.scales.down_b);
                         if constexpr(MODE == NS_UPDATE)
                         {
                             h8 low;
@@ -887,7 +936,7 @@ namespace
                             d[q] = v;
                             v    = 0.f;
                         }
-                        mine[i][j][r] = (_Float16)(v * UP);
+                        mine[i][j][r] = (_Float16)(v * a.scales.up_a);
                     }
                     *(h4*)&A[q * PA + p] = mine[i][j]; // (symmetric)
                 }
@@ -927,14 +976,14 @@ namespace
 #pragma unroll
                     for(int r = 0; r < 4; r++)
                     {
-                        const float off = (float)mine[i][j][r] * DOWN;
-                        float       v = cb * off + cc * (acc[i][j][r] * (DOWN * DOWN) + (dp[r] + dq) * off);
+                        const float off = (float)mine[i][j][r] * a.scales.down_a;
+                        float       v = cb * off + cc * (acc[i][j][r] * (a.scales.down_a * a.scales.down_a) + (dp[r] + dq) * off);
                         if(p + r == q)
                         {
                             e[q] = v + cb * dq + cc * dq * dq;
                             v    = 0.f;
                         }
-                        out[r] = (_Float16)(v * UP);
+                        out[r] = (_Float16)(v * a.scales.up_b);
                     }
                     *(h4*)&A[q * PA + p] = out;
                 }
@@ -945,7 +994,7 @@ namespace
 #pragma unroll
             for(int j = 0; j < UJ; j++)
             {
-                const float f = (ca + e[16 * (uj + j) + fr]) * UP;
+                const float f = (ca + e[16 * (uj + j) + fr]) * a.scales.up_b;
 #pragma unroll
                 for(int i = 0; i < UI; i++)
                 {
@@ -1018,7 +1067,7 @@ namespace
             for(int i = 0; i < UI; i++)
 #pragma unroll
                 for(int j = 0; j < UJ; j++)
-                    x[i][j] *= DOWN;
+                    x[i][j] *= a.scales.down_b;
             __syncthreads(); // (X_hi, X_lo, B' and e have been read)
             if(step + 1 < steps)
             {
@@ -1284,6 +1333,7 @@ extern "C" int hiptk_orthogonalize(const hiptk_orthogonalize_t* p, void* workspa
     a.type_x            = p->type_x;
     a.type_o            = p->type_o;
     a.epsilon           = p->epsilon;
+    a.scales            = scales_of(p->coefficients, p->steps);
     if(is_small(p))
     {
         Coefficients c;

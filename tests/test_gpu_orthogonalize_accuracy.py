@@ -69,3 +69,29 @@ def test_steps_that_converge(gpu_handle, rows, cols):
     for steps in (16, 17, 30):
         got, want = L.gpu_orthogonalize(gpu_handle, x, "f32", "f16", steps, coefficients * steps), L.orthogonalize_plain(x, steps, coefficients * steps)
         assert L.relative(got, want) <= 3e-3 + L.ROUND["f16"][0], steps
+
+
+# steps whose A or B has entries of 64 and more, while no singular value of an iterate reaches 16
+GROWING = {"A of up to 225": [15.0, 0.0, 0.0, 1.0, -0.01, 1e-5], "B of up to 130": [-118.0, 130.0, 0.0],
+           "A back to 1": [15.0, 0.0, 0.0, 1.0 / 15, 0.0, 0.0, 1.5, -0.5, 0.0]}
+
+
+@pytest.mark.parametrize("rows,cols", [(2, 4), (64, 64), (128, 256), (100, 20), (2, 600), (600, 2), (33, 600), (300, 200)])
+@pytest.mark.parametrize("name", GROWING)
+def test_coefficients_that_grow(gpu_handle, rows, cols, name):
+    """Of equal entries, so that A and B have entries near their singular value: the tolerance follows that one value s.  X_hi, A' and B' are rounded by up to
+    2^-11 of themselves, all entries alike; X_hi is four times in A A X and twice in A X beside the X that B multiplies, A' twice and once, B' once."""
+    coefficients = GROWING[name]
+    x = torch.full((2, rows, cols), 0.37)
+    s, off, u = 1.0, 0.0, 2.0**-11
+    for i in range(0, len(coefficients), 3):
+        a, b, c = coefficients[i:i + 3]
+        grown = abs(a + 3 * b * s**2 + 5 * c * s**4) * off + u * (5 * abs(b) * s**3 + 8 * abs(c) * s**5)
+        s, off = a * s + b * s**3 + c * s**5, grown
+        assert abs(s) < 16
+    steps = len(coefficients) // 3
+    want = L.orthogonalize_plain(x, steps, coefficients)
+    assert abs(float(want[0, 0, 0]) - s / (rows * cols)**0.5) < 1e-3 * abs(s)
+    for out in ("bf16", "f16"):
+        got = L.gpu_orthogonalize(gpu_handle, x, "f32", out, steps, coefficients)
+        assert L.relative(got, want) <= off / abs(s) + L.ROUND[out][0], (s, off)
