@@ -868,7 +868,8 @@ namespace
         // (neither is faster than B comes from memory, and where both are as fast as that the registers are)
         const double floor = 5.0 + (double)p->N * (double)p->K / 4.8e6;
         best               = best < floor ? floor : best;
-        for(int tm = 1; tm <= 2 && p->M <= FEW; tm++)
+        const bool fits    = (p->N + 15) / 16 * 512 < (1ll << 31); // (threads of the grid in x)
+        for(int tm = 1; tm <= 2 && p->M <= FEW && fits; tm++)
         {
             const int64_t beside = (((p->M + 16 * tm - 1) / (16 * tm)) * ((p->N + 15) / 16) + UNITS - 1) / UNITS;
             double        us     = 6.5 + (double)nk * few_cost(p->M, tm, beside, wide);
