@@ -379,7 +379,7 @@ extern "C" int hiptensorAmdOrthogonalizeGetWorkspaceSize(
         p.cols                  = cols;
         p.type_x                = class_of(typeX);
         p.type_o                = class_of(typeO);
-        p.steps                 = 1;
+        p.steps                 = INT32_MAX; // (enough for any number)
         *workspaceSize          = hiptk_orthogonalize_workspace_bytes(&p);
         return HIPTENSOR_STATUS_SUCCESS;
     });

@@ -1285,7 +1285,7 @@ extern "C" const char* hiptk_orthogonalize_kernel_name(const hiptk_orthogonalize
 
 extern "C" uint64_t hiptk_orthogonalize_workspace_bytes(const hiptk_orthogonalize_t* p)
 {
-    if(!well_formed(p) || p->batch == 0 || p->rows == 0 || p->cols == 0)
+    if(!well_formed(p) || p->batch == 0 || p->rows == 0 || p->cols == 0 || is_small(p))
         return 0;
     const Layout l = layout_of(p);
     return (uint64_t)(l.per * p->batch + l.sums);
@@ -1301,7 +1301,8 @@ extern "C" int hiptk_orthogonalize(const hiptk_orthogonalize_t* p, void* workspa
         return HIPTK_OK;
     if(!p->X || !p->O)
         return HIPTK_ERR_ARG;
-    if(!workspace || workspace_bytes < hiptk_orthogonalize_workspace_bytes(p) || ((uintptr_t)workspace & 255))
+    const uint64_t need = hiptk_orthogonalize_workspace_bytes(p);
+    if(need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255)))
         return HIPTK_ERR_WORKSPACE;
     const Layout l      = layout_of(p);
     char*        ws     = (char*)workspace;

@@ -278,7 +278,8 @@ int hiptensorAmdBlockScaledProduct(const void*  handle,
  * the exact iteration's for up to 6 steps and 6e-3 for up to 12; four times that where the shorter side is below 16 or entries or rows repeat, so that
  * roundings do not average out; and 2^-23 * 3.4445^steps more where X lacks directions (2e-4 after 6 steps, 3e-2 after 10), since each step multiplies
  * what rounding leaves there.  The iterates' singular values must stay below 16, which the default coefficients guarantee (A and B have whatever size follows).  O may be X where the types' sizes
- * and the layouts agree.  The workspace (256-byte aligned) is required in full. */
+ * and the layouts agree.  The workspace (256-byte aligned) is required in full; GetWorkspaceSize says how much is enough for
+ * any number of steps.  Matrices of up to 64 x 512 or 128 x 256 (or turned) with up to 16 steps need none: null is accepted there. */
 int hiptensorAmdOrthogonalizeGetWorkspaceSize(
     const void* handle, int64_t batch, int64_t rows, int64_t cols, int typeX, int typeO, uint64_t* workspaceSize);
 int hiptensorAmdOrthogonalize(const void*  handle,

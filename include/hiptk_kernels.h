@@ -338,6 +338,7 @@ typedef struct hiptk_orthogonalize
     const float* coefficients;
 } hiptk_orthogonalize_t;
 const char* hiptk_orthogonalize_kernel_name(const hiptk_orthogonalize_t* prob);
+/* Bytes of workspace, 256-byte aligned, that the problem's number of steps needs (none where one workgroup holds a matrix). */
 uint64_t    hiptk_orthogonalize_workspace_bytes(const hiptk_orthogonalize_t* prob);
 int         hiptk_orthogonalize(const hiptk_orthogonalize_t* prob, void* workspace, uint64_t workspace_bytes, void* stream, int* hip_error);
 

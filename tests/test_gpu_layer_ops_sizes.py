@@ -28,3 +28,12 @@ def test_one_token_and_more_columns_than_a_grid_of_few_tokens_holds(gpu_handle):
         terms = b[rows].view(torch.float8_e4m3fn).float() * va * scale[:, None]
         want, most = terms.sum(1), terms.abs().sum(1)
         assert ((d[0, rows].float() - want).abs() <= 2.0**-8 * want.abs() + 2.0**-10 * most).all(), at
+
+
+def test_small_orthogonalisation_without_a_workspace(gpu_handle):
+    x = torch.randn(3, 60, 200, generator=torch.Generator().manual_seed(4))
+    want = L.gpu_orthogonalize(gpu_handle, x, "f32")
+    dx, o = x.cuda(), torch.empty(3, 60, 200, dtype=torch.bfloat16, device="cuda")
+    api.check(api.hiptensorOrthogonalize(gpu_handle, 3, 60, 200, dx.data_ptr(), api.HIP_R_32F, 200, 12000, 5, None, 1e-7, o.data_ptr(), api.HIP_R_16BF, 200,
+                                         12000, None, 0, L.stream()))
+    assert torch.equal(o.cpu(), want)
