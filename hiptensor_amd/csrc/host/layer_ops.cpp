@@ -226,7 +226,7 @@ extern "C" int hiptensorAmdBlockQuantize(const void* handle,
         if(off(X, bytes_of(typeX)) || off(S, 4) || off(ST, 4))
             return refuse(fn, HIPTENSOR_STATUS_INVALID_VALUE, "Input Parameter Error : an address is no multiple of its element's size");
         if(blocks(rows, 128) * blocks(cols, 128) > MOST / 256)
-            return refuse(fn, HIPTENSOR_STATUS_NOT_SUPPORTED, "A matrix of more than 2^23 tiles of 128 x 128 is not supported");
+            return refuse(fn, HIPTENSOR_STATUS_NOT_SUPPORTED, "A matrix of 2^23 tiles of 128 x 128 or more is not supported");
         Handle* h = nullptr;
         if(auto st = device_of(fn, handle, h); st != HIPTENSOR_STATUS_SUCCESS)
             return st;
@@ -329,7 +329,7 @@ extern "C" int hiptensorAmdBlockScaledProduct(const void*  handle,
         if(off(SA, 4) || off(SB, 4) || off(D, bytes_of(typeD)) || (*beta != 0.f && off(C, bytes_of(typeD))))
             return refuse(fn, HIPTENSOR_STATUS_INVALID_VALUE, "Input Parameter Error : an address is no multiple of its element's size");
         if(blocks(M, 64) * blocks(N, 64) > MOST / 256)
-            return refuse(fn, HIPTENSOR_STATUS_NOT_SUPPORTED, "A result of more than 2^23 tiles of 64 x 64 is not supported");
+            return refuse(fn, HIPTENSOR_STATUS_NOT_SUPPORTED, "A result of 2^23 tiles of 64 x 64 or more is not supported");
         Handle* h = nullptr;
         if(auto st = device_of(fn, handle, h); st != HIPTENSOR_STATUS_SUCCESS)
             return st;

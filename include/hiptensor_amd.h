@@ -207,8 +207,10 @@ int64_t hiptensorAmdPlanTable(const void* plan, int which, int32_t* out, int64_t
  *
  * Status codes: NOT_INITIALIZED (a handle or needed pointer is null), INVALID_VALUE (a
  * negative or too large extent, a leading dimension below its row, an address that is no multiple of its element),
- * NOT_SUPPORTED (a data type or block shape there is no kernel for), INSUFFICIENT_WORKSPACE, ARCH_MISMATCH (a handle
- * without a device, or another current device), EXECUTION_FAILED (the launch failed).  Extents are at most 2^31 - 256.
+ * NOT_SUPPORTED (a data type or block shape there is no kernel for, or too many tiles), INSUFFICIENT_WORKSPACE, ARCH_MISMATCH (a handle
+ * without a device, or another current device), EXECUTION_FAILED (the launch failed).
+ * Limits: extents of the quantisation and of the product at most 2^31 - 256, the former's matrix fewer than 2^23 tiles of 128 x 128, the latter's
+ * result fewer than 2^23 of 64 x 64; the orthogonalisation's batch at most 65535, its matrices' shorter side 2^16, the longer one 2^20.
  * An empty result returns SUCCESS without a launch.
  * ------------------------------------------------------------------------------------------ */
 

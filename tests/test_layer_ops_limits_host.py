@@ -40,3 +40,25 @@ def test_matrices_of_one_workgroup_need_no_workspace(host_handle):
         assert need > 0 and call(rows, cols, 17, None, 0) == call(rows, cols, 17, 1 << 20, need - 1) == small and call(rows, cols, 17, 1 << 20, need) == ok
     for rows, cols in ((65, 257), (64, 513), (129, 129)):
         assert call(rows, cols, 5, None, 0) == small
+
+
+def test_largest_sizes_that_the_header_names(host_handle):
+    """Accepted at the limit (as far as a handle without a device goes), refused one beyond it."""
+    ok, invalid, unsupported = api.HIPTENSOR_STATUS_ARCH_MISMATCH, api.HIPTENSOR_STATUS_INVALID_VALUE, api.HIPTENSOR_STATUS_NOT_SUPPORTED
+    at, most, tiles = 1 << 20, (1 << 31) - 256, (1 << 23) - 1
+
+    def quantize(rows, cols):
+        return api.hiptensorBlockQuantize(host_handle, rows, cols, at, api.HIP_R_16BF, cols, 1, at, cols, at, rows, None, 0, None, 0, None)
+
+    def product(m, n, k):
+        return api.hiptensorBlockScaledProduct(host_handle, m, n, k, 1.0, at, k, at, m, at, k, at, n, 1, 0.0, None, at, api.HIP_R_32F, n, None, 0, None)
+
+    def orthogonalize(batch, rows, cols):
+        return api.hiptensorOrthogonalize(host_handle, batch, rows, cols, at, api.HIP_R_32F, cols, rows * cols, 5, None, 0.0, at, api.HIP_R_16F, cols,
+                                          rows * cols, at << 20, 1 << 60, None)
+
+    assert quantize(1, tiles * 128) == ok and quantize(1, tiles * 128 + 129) == unsupported and quantize(most + 1, 1) == invalid
+    assert product(1, tiles * 64, 8) == ok and product(1, tiles * 64 + 65, 8) == unsupported and product(8, 8, most) == ok and product(8, 8, most + 1) == invalid
+    assert orthogonalize(65535, 100, 200) == ok and orthogonalize(65536, 100, 200) == invalid
+    assert orthogonalize(1, 1 << 16, 1 << 20) == orthogonalize(1, 1 << 20, 1 << 16) == ok
+    assert orthogonalize(1, (1 << 16) + 1, 1 << 20) == orthogonalize(1, 1, (1 << 20) + 1) == invalid
