@@ -26,6 +26,8 @@
 // which every step keeps zero.
 #include <hip/hip_runtime.h>
 
+#include <array>
+#include <string>
 #include <type_traits>
 #include <utility>
 
@@ -1278,9 +1280,23 @@ namespace
     }
 }
 
+// newton_schulz_products and the tiles of square (or "sliced"), mix and update; "64r2" is the tile of 64 with two stages
 extern "C" const char* hiptk_orthogonalize_kernel_name(const hiptk_orthogonalize_t* p)
 {
-    return !well_formed(p) ? "" : is_small(p) ? "newton_schulz_small" : "newton_schulz_products";
+    if(!well_formed(p) || p->batch == 0 || p->rows == 0 || p->cols == 0)
+        return "";
+    if(is_small(p))
+        return "newton_schulz_small";
+    static const auto names = [] {
+        const char*                                              tile[TILES + 1] = {"256", "192", "128", "64", "64r2", "sliced"};
+        std::array<std::string, (TILES + 1) * TILES * TILES> all;
+        for(int i = 0; i < (int)all.size(); i++)
+            all[i] = std::string("newton_schulz_products_") + tile[i / (TILES * TILES)] + "_" + tile[i / TILES % TILES] + "_" + tile[i % TILES];
+        return all;
+    }();
+    const Layout l = layout_of(p);
+    const int    square = l.slices > 1 ? TILES : choice_of(NS_SQUARE, l.m, l.n, p->batch);
+    return names[(square * TILES + choice_of(NS_MIX, l.m, l.n, p->batch)) * TILES + choice_of(NS_UPDATE, l.m, l.n, p->batch)].c_str();
 }
 
 extern "C" uint64_t hiptk_orthogonalize_workspace_bytes(const hiptk_orthogonalize_t* p)
