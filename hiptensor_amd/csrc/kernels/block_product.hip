@@ -15,14 +15,16 @@
 #include <hip/hip_runtime.h>
 
 #include <type_traits>
-#include <utility>
 
 #include "dma_lds.hpp"
 #include "hd_addr.hpp"
 #include "hiptk_kernels.h"
+#include "tile_walk.hpp"
 
 namespace
 {
+    using hiptk::each;
+
     typedef int   v8i __attribute__((ext_vector_type(8)));
     typedef float v4f __attribute__((ext_vector_type(4)));
 
@@ -252,13 +254,6 @@ namespace
 
     // ---- tiles loaded straight into LDS ------------------------------------------------------------------------------
 
-    __device__ __forceinline__ void barrier()
-    {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    }
-
     // The slice of K that a workgroup of a split launch takes: its blocks of the operands and scales, its part of the sums
     __device__ __forceinline__ void slice_of(PArgs& a, uint32_t slice)
     {
@@ -274,30 +269,6 @@ namespace
         a.alpha            = 1.f;
         a.beta             = 0.f;
         a.type             = HIPTK_F32;
-    }
-
-    // f(integral_constant<int, 0>) ... f(integral_constant<int, N - 1>): what indexes registers must be a constant
-    template <typename F, int... I>
-    __device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>)
-    {
-        (f(std::integral_constant<int, I>{}), ...);
-    }
-    template <int N, typename F>
-    __device__ __forceinline__ void each(F&& f)
-    {
-        each_impl(f, std::make_integer_sequence<int, N>{});
-    }
-
-    // Tile of this workgroup: the dies (XCDs, workgroup ids congruent mod 8) take contiguous ranges, walked in groups of 4 rows of tiles
-    __device__ __forceinline__ void tile_of(const PArgs& a, int& tm, int& tn)
-    {
-        const uint32_t tiles = (uint32_t)a.tiles_m * (uint32_t)a.tiles_n, wg = blockIdx.x;
-        const uint32_t xcd = wg & 7, nth = wg >> 3, base = tiles >> 3, rem = tiles & 7;
-        const uint32_t lin  = xcd * base + (xcd < rem ? xcd : rem) + nth;
-        const uint32_t band = 4u * (uint32_t)a.tiles_n, g = lin / band, first = g * 4;
-        const uint32_t rows = (uint32_t)a.tiles_m - first < 4 ? (uint32_t)a.tiles_m - first : 4, r = lin - g * band;
-        tm                  = (int)(first + r % rows);
-        tn                  = (int)(r / rows);
     }
 
     // BM x BN on WM x WN wavefronts, a wavefront NJ x NI blocks of 16 x 16.  A ring of ST LDS stages of one block of K each; rows of 128 codes, the
@@ -336,7 +307,7 @@ namespace
         const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
         const int wm = wave % WM, wn = wave / WM;
         int       tm, tn;
-        tile_of(a, tm, tn);
+        hiptk::tile_of(hiptk::place_of(blockIdx.x, (uint32_t)a.tiles_m * (uint32_t)a.tiles_n), a.tiles_m, a.tiles_n, tm, tn);
         const int m0 = tm * BM, n0 = tn * BN;
 
         // what each lane loads: rows beyond the last read the last one
@@ -490,7 +461,7 @@ namespace
                     *q = x;
                 }
             __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_lgkm0);
-            barrier();
+            hiptk::lds_barrier();
         };
         // loads FROM .. TO - 1 of stage t into slot s, all at once
         auto load_all = [&](int t, int s, auto from_c, auto to_c) __attribute__((always_inline)) {
@@ -519,7 +490,7 @@ namespace
                     {
                         // (loads complete in order: those of the stages behind t + 1 may be under way)
                         __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_vm_lgkm0(REST ? (ST - 2) * T::LOADS : 0));
-                        barrier();
+                        hiptk::lds_barrier();
                         if(!MORE && tail && t + 1 == nk - 1)
                             clear_tail(next);
                         if(MORE && tail && t + ST == nk - 1)
@@ -585,7 +556,7 @@ namespace
         }
         else
             __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_vm_lgkm0(0));
-        barrier();
+        hiptk::lds_barrier();
         if(tail && nk == 1)
             clear_tail(0);
         fetch_a(stage_at(0), First{});
@@ -607,7 +578,7 @@ namespace
         // Results pass through LDS, 16 rows at a time and within the wavefront, so that D is written (and C read) in whole lines:
         // stored as the accumulators lie, 32 bytes in each of 16 rows, a compute unit wrote 8 bytes a cycle.  C's rows are asked for a group
         // ahead: D may be C, so no load passes a store, and asked for where they are added each would be waited for.
-        barrier(); // (every wavefront is done with the last stage)
+        hiptk::lds_barrier(); // (every wavefront is done with the last stage)
         float* stage = (float*)lds + wave * 16 * (NI * 16 + 4);
         auto   store = [&](auto type, auto add_c) __attribute__((always_inline)) {
             constexpr bool                     ADD = decltype(add_c)::value;

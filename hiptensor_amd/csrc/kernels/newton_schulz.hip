@@ -29,14 +29,16 @@
 #include <array>
 #include <string>
 #include <type_traits>
-#include <utility>
 
 #include "dma_lds.hpp"
 #include "hd_addr.hpp"
 #include "hiptk_kernels.h"
+#include "tile_walk.hpp"
 
 namespace
 {
+    using hiptk::each;
+
     typedef _Float16 h8 __attribute__((ext_vector_type(8)));
     typedef _Float16 h4 __attribute__((ext_vector_type(4)));
     typedef float    f4 __attribute__((ext_vector_type(4)));
@@ -288,41 +290,6 @@ namespace
         tj = 4 * g + c;
     }
 
-    template <typename F, int... I>
-    __device__ __forceinline__ void each_impl(F&& f, std::integer_sequence<int, I...>)
-    {
-        (f(std::integral_constant<int, I>{}), ...);
-    }
-    template <int N, typename F>
-    __device__ __forceinline__ void each(F&& f)
-    {
-        each_impl(f, std::make_integer_sequence<int, N>{});
-    }
-
-    __device__ __forceinline__ void barrier()
-    {
-        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
-        __builtin_amdgcn_s_barrier();
-        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
-    }
-
-    // The tiles of all matrices are one list, matrix after matrix; the dies (workgroup ids congruent mod 8, an L2 each) take contiguous ranges of
-    // it, so that an L2 holds one or two of a batch's matrices at a time (X X^T of 12 x 1024 x 1024: 32 us with
-    // workgroups dealt round the dies, 24 us so).
-    __device__ __forceinline__ uint32_t place_of(uint32_t wg, uint32_t all)
-    {
-        const uint32_t xcd = wg & 7, nth = wg >> 3, base = all >> 3, rem = all & 7;
-        return xcd * base + (xcd < rem ? xcd : rem) + nth;
-    }
-    // tile `lin` of a plane of tiles_p x tiles_q, walked in groups of 4 rows
-    __device__ __forceinline__ void tile_of(uint32_t lin, int tiles_p, int tiles_q, int& tp, int& tq)
-    {
-        const uint32_t band = 4u * (uint32_t)tiles_q, g = lin / band, first = g * 4;
-        const uint32_t rows = (uint32_t)tiles_p - first < 4 ? (uint32_t)tiles_p - first : 4, r = lin - g * band;
-        tp                  = (int)(first + r % rows);
-        tq                  = (int)(r / rows);
-    }
-
     // One product P Q^T of a step, BP x BQ outputs a workgroup on WP x WQ wavefronts, NI x NJ blocks of 16 x 16 each, k in stages of 64 through a ring
     // of ST in LDS (rows of 128 bytes; the 16-byte chunk at position c of a row holds chunk c ^ (row / 2) % 8).
     // 8192 x 4096: square 120 us on tiles of 192 (MFMAs 76 % of the busy cycles), mix 71, update 239 on tiles of 256 (63 %, and 670 MB that it
@@ -373,10 +340,10 @@ namespace
         const int      wp = wave % WP, wq = wave / WP;
         int            ti, tj;
         const uint32_t tiles_q = (uint32_t)((a.m + BQ - 1) / BQ), tiles_p = (uint32_t)((a.n + BP - 1) / BP);
-        const uint32_t tiles = UPDATE ? tiles_p * tiles_q : tiles_q * (tiles_q + 1) / 2, place = place_of(blockIdx.x, gridDim.x);
+        const uint32_t tiles = UPDATE ? tiles_p * tiles_q : tiles_q * (tiles_q + 1) / 2, place = hiptk::place_of(blockIdx.x, gridDim.x); // (the tiles of all matrices are one list, matrix after matrix)
         const uint32_t z = place / tiles;
         if(UPDATE)
-            tile_of(place - z * tiles, (int)tiles_p, (int)tiles_q, ti, tj);
+            hiptk::tile_of(place - z * tiles, (int)tiles_p, (int)tiles_q, ti, tj);
         else
             triangle((int)(place - z * tiles), (int)tiles_q, ti, tj);
         const int rows_p = UPDATE ? a.n : a.m, K = SQUARE ? a.n : a.m;
@@ -571,7 +538,7 @@ namespace
             if constexpr(FOLLOWS)
             {
                 __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_vm_lgkm0(MORE ? (ST - 2) * T::LOADS : 0));
-                barrier();
+                hiptk::lds_barrier();
             }
             kstep(Second{}, lds + next * T::STAGE, follows_c, t + ST, slot, more_c);
             slot = next;
@@ -598,7 +565,7 @@ namespace
                 __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_vm_lgkm0((ST - 1) * T::LOADS));
             else
                 __builtin_amdgcn_s_waitcnt(hiptk::waitcnt_vm_lgkm0(0));
-            barrier();
+            hiptk::lds_barrier();
             each<NF>([&](auto u_c) __attribute__((always_inline)) { fetch(lds, First{}, u_c); });
             int t = 0;
             for(; t + ST < nk; t++)
@@ -623,7 +590,7 @@ namespace
         // go through `rows` as f32 rows of W consecutive p; a lane then holds eight p of one q, reads the elementwise terms (a column group
         // ahead), and stores along p.  The other orientation (the mirrored half of a symmetric matrix, O of a tall X) is stored
         // every 32 q from `turn`, by transposing reads that hand a lane four consecutive q of one p.
-        barrier(); // (every wavefront is done with the last stage)
+        hiptk::lds_barrier(); // (every wavefront is done with the last stage)
         float*    rows = (float*)(lds + wave * T::PASS);
         uint16_t* turn = (uint16_t*)(lds + wave * T::PASS + 16 * PR * 4);
         if constexpr(!EARLY)
