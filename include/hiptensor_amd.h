@@ -279,7 +279,7 @@ int hiptensorAmdBlockScaledProduct(const void*  handle,
  * HIP_R_16BF or HIP_R_32F; typeO: HIP_R_16F or HIP_R_16BF.  The products are of f16 with f32 sums; the iterate is held in
  * 22 bits and the diagonals of A and B in f32.  With the default coefficients and before O's rounding, that keeps the result within 3e-3 (2-norm) of
  * the exact iteration's for up to 6 steps and 6e-3 for up to 12; four times that where the shorter side is below 16 or entries or rows repeat, so that
- * roundings do not average out; and 2^-23 * 3.4445^steps more where X lacks directions (2e-4 after 6 steps, 3e-2 after 10), since each step multiplies
+ * roundings do not average out; and 2^-22 * 3.4445^steps more where X lacks directions (4e-4 after 6 steps, 6e-2 after 10), since each step multiplies
  * what rounding leaves there.  The iterates' singular values must stay below 16, which the default coefficients guarantee (A and B have whatever size follows).  O may be X where the types' sizes
  * and the layouts agree.  The workspace (256-byte aligned) is required in full; GetWorkspaceSize says how much is enough for
  * any number of steps.  Matrices of up to 64 x 512 or 128 x 256 (or turned) with up to 16 steps need none: null is accepted there. */

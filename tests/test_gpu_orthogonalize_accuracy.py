@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 
 
 def bound(rows, cols, steps, repeats, out):
-    """The error that the header allows, and one rounding to the result's type."""
+    """The error that the header allows (with 2^-23 for what directions that X lacks get, half of the header's), and one rounding to the result's type."""
     base = 3e-3 if steps <= 6 else 6e-3
     few = 4 if repeats or min(rows, cols) < 16 else 1
     return base * few + 2.0**-23 * L.COEFFICIENTS[0]**steps + L.ROUND[out][0]
